@@ -100,13 +100,18 @@ def quantize_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return codes, scale
 
 
+def _for_backward(num: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The counts as they are now: the next dispatch writes its own into the same tensor, maybe before this step's backward."""
+    return None if num is None else num.clone()
+
+
 class _Matmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, expert_x, weight, expert_num_tokens, expert_padding, tokens_per_expert):
         out = expert_x.new_zeros((expert_x.shape[0], weight.shape[1]))
         expert_matmul(out, expert_x, weight, expert_num_tokens, expert_padding=expert_padding,
                       tokens_per_expert=tokens_per_expert)
-        ctx.save_for_backward(expert_x, weight, expert_num_tokens)
+        ctx.save_for_backward(expert_x, weight, _for_backward(expert_num_tokens))
         ctx.expert_padding = expert_padding
         return out
 
@@ -127,7 +132,7 @@ class _Gated(torch.autograd.Function):
         projections = expert_x.new_empty((expert_x.shape[0], weight.shape[1]))
         expert_gated(out, expert_x, weight, expert_num_tokens, projections=projections, expert_padding=expert_padding,
                      tokens_per_expert=tokens_per_expert)
-        ctx.save_for_backward(expert_x, weight, expert_num_tokens, projections)
+        ctx.save_for_backward(expert_x, weight, _for_backward(expert_num_tokens), projections)
         ctx.expert_padding = expert_padding
         return out
 

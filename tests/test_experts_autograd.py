@@ -1,0 +1,96 @@
+"""The experts' products for autograd without a GPU: plain products stand in for the library's calls.  They write past torch's
+record of a tensor's versions, as the library does, and refuse what it refuses."""
+
+import pytest
+import torch
+
+import experts_reference as ref
+from pplx_garden_amd.kernels import experts
+
+
+def _rows(num, padding, x, weight):
+    counts = [x.shape[0]] if num is None else num.tolist()
+    assert len(counts) == weight.shape[0]
+    return [slice(first, first + count) for first, count in ref.ranges(counts, padding, x.shape[0])]
+
+
+def _aligned(*tensors):
+    for t in tensors:
+        if t is not None and t.data_ptr() % 16 != 0:
+            raise RuntimeError("must be multiples of 16 bytes")
+
+
+def _halves(p):
+    return p.double().chunk(2, -1)
+
+
+@pytest.fixture(autouse=True)
+def plain_calls(monkeypatch):
+    def expert_matmul(out, x, w, num=None, expert_x_scale=None, weight_scale=None, expert_padding=1, tokens_per_expert=None):
+        _aligned(out, x, w)
+        for e, at in enumerate(_rows(num, expert_padding, x, w)):
+            out.data[at] = (x[at].double() @ w[e].double().T).to(out.dtype)
+
+    def expert_gated(out, x, w, num=None, expert_x_scale=None, weight_scale=None, out_scale=None, projections=None,
+                     expert_padding=1, tokens_per_expert=None):
+        expert_matmul(projections, x, w, num, expert_padding=expert_padding)
+        g, u = _halves(projections)
+        for at in _rows(num, expert_padding, x, w):
+            out.data[at] = (ref.silu(g[at]) * u[at]).to(out.dtype)
+
+    def expert_matmul_grad(grad_x, grad_w, grad_out, x, w, num=None, expert_padding=1):
+        _aligned(grad_x, grad_w, grad_out, x, w)
+        for e, at in enumerate(_rows(num, expert_padding, x, w)):
+            if grad_x is not None:
+                grad_x.data[at] = (grad_out[at].double() @ w[e].double()).to(grad_x.dtype)
+            if grad_w is not None:
+                grad_w.data[e] = (grad_out[at].double().T @ x[at].double()).to(grad_w.dtype)
+
+    def expert_gated_grad(grad_x, grad_w, grad_projections, grad_out, projections, x, w, num=None, expert_padding=1):
+        _aligned(grad_out)
+        d = torch.cat(ref.gate_gradient(grad_out.double(), *_halves(projections)), -1)
+        grad_projections.data.copy_(d.to(grad_projections.dtype))
+        expert_matmul_grad(grad_x, grad_w, grad_projections, x, w, num, expert_padding)
+
+    for call in (expert_matmul, expert_gated, expert_matmul_grad, expert_gated_grad):
+        monkeypatch.setattr(experts, call.__name__, call)
+
+
+def _layer(x, w1, w2, num):
+    return experts.matmul(experts.gated(x, w1, num), w2, num)
+
+
+def _operands(counts=(4, 0), n=16, k=24):
+    gen = torch.Generator().manual_seed(0)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=gen).bfloat16()
+
+    num = torch.tensor(counts, dtype=torch.int32)
+    rows = int(num.sum())
+    return normal(rows, k), normal(len(counts), 2 * n, k), normal(len(counts), k, n), num, normal(rows, k)
+
+
+def _gradients(x, w1, w2, num, grad_y, between=None):
+    leaves = [t.clone().requires_grad_() for t in (x, w1, w2)]
+    y = _layer(*leaves, num)
+    if between is not None:
+        between()
+    y.backward(grad_y)
+    return [t.grad for t in leaves]
+
+
+def test_backward_uses_the_counts_of_its_own_forward():
+    """Dispatch writes the next step's counts into the same tensor before the first step's backward."""
+    x, w1, w2, num, grad_y = _operands()
+    want = _gradients(x, w1, w2, num, grad_y)
+    assert (want[1][0] != 0).any() and (want[1][1] == 0).all()
+    got = _gradients(x, w1, w2, num, grad_y, between=lambda: num.data.copy_(torch.tensor([0, 4])))
+    assert num.tolist() == [0, 4]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_a_dense_product_keeps_no_counts():
+    x, w1, w2, _, grad_y = _operands((4,))
+    assert [g.shape for g in _gradients(x, w1, w2, None, grad_y)] == [x.shape, w1.shape, w2.shape]
