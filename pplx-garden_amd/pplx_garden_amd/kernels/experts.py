@@ -100,9 +100,21 @@ def quantize_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return codes, scale
 
 
-def _for_backward(num: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """The counts as they are now: the next dispatch writes its own into the same tensor, maybe before this step's backward."""
-    return None if num is None else num.clone()
+def _save_for_backward(ctx, expert_x, weight, num, padding, *more) -> None:
+    """The rows are read by the weight's gradient alone and the weight by that of the rows: what no gradient reads is not kept, and may
+    change.  The counts are copied: the next dispatch writes its own into the same tensor, maybe before this step's backward."""
+    ctx.save_for_backward(expert_x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None,
+                          None if num is None else num.clone(), *more)
+    ctx.shapes, ctx.expert_padding = (expert_x.shape, weight.shape), padding
+
+
+def _gradients(ctx, grad_out):
+    """Memory for both gradients (None: not asked for), the operands, and what else was saved.  In the place of an operand that was not
+    kept stands the gradient that is as large: the calls do not read its values."""
+    expert_x, weight, *more = ctx.saved_tensors
+    grad_x = grad_out.new_zeros(ctx.shapes[0]) if ctx.needs_input_grad[0] else None
+    grad_w = grad_out.new_empty(ctx.shapes[1]) if ctx.needs_input_grad[1] else None
+    return grad_x, grad_w, grad_x if expert_x is None else expert_x, grad_w if weight is None else weight, *more
 
 
 class _Matmul(torch.autograd.Function):
@@ -111,16 +123,13 @@ class _Matmul(torch.autograd.Function):
         out = expert_x.new_zeros((expert_x.shape[0], weight.shape[1]))
         expert_matmul(out, expert_x, weight, expert_num_tokens, expert_padding=expert_padding,
                       tokens_per_expert=tokens_per_expert)
-        ctx.save_for_backward(expert_x, weight, _for_backward(expert_num_tokens))
-        ctx.expert_padding = expert_padding
+        _save_for_backward(ctx, expert_x, weight, expert_num_tokens, expert_padding)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        expert_x, weight, num = ctx.saved_tensors
-        grad_x = torch.zeros_like(expert_x, memory_format=torch.contiguous_format) if ctx.needs_input_grad[0] else None
-        grad_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if ctx.needs_input_grad[1] else None
+        grad_x, grad_w, expert_x, weight, num = _gradients(ctx, grad_out)
         expert_matmul_grad(grad_x, grad_w, grad_out.contiguous(), expert_x, weight, num, ctx.expert_padding)
         return grad_x, grad_w, None, None, None
 
@@ -132,16 +141,13 @@ class _Gated(torch.autograd.Function):
         projections = expert_x.new_empty((expert_x.shape[0], weight.shape[1]))
         expert_gated(out, expert_x, weight, expert_num_tokens, projections=projections, expert_padding=expert_padding,
                      tokens_per_expert=tokens_per_expert)
-        ctx.save_for_backward(expert_x, weight, _for_backward(expert_num_tokens), projections)
-        ctx.expert_padding = expert_padding
+        _save_for_backward(ctx, expert_x, weight, expert_num_tokens, expert_padding, projections)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        expert_x, weight, num, projections = ctx.saved_tensors
-        grad_x = torch.zeros_like(expert_x, memory_format=torch.contiguous_format) if ctx.needs_input_grad[0] else None
-        grad_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if ctx.needs_input_grad[1] else None
+        grad_x, grad_w, expert_x, weight, num, projections = _gradients(ctx, grad_out)
         expert_gated_grad(grad_x, grad_w, torch.empty_like(projections), grad_out.contiguous(), projections, expert_x, weight,
                           num, ctx.expert_padding)
         return grad_x, grad_w, None, None, None

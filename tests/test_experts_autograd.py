@@ -94,3 +94,34 @@ def test_backward_uses_the_counts_of_its_own_forward():
 def test_a_dense_product_keeps_no_counts():
     x, w1, w2, _, grad_y = _operands((4,))
     assert [g.shape for g in _gradients(x, w1, w2, None, grad_y)] == [x.shape, w1.shape, w2.shape]
+
+
+@pytest.mark.parametrize("call", ["matmul", "gated"])
+@pytest.mark.parametrize("frozen", ["weight", "rows"])
+def test_only_what_a_gradient_needs_has_to_stay_as_it_was(call, frozen):
+    """Gradients of the rows do not read the rows, nor those of a weight the weight: with one of them frozen the other's values may change
+    before backward."""
+    x, w1, _, num, _ = _operands((2, 3))
+    grad_y = torch.randn((5, w1.shape[1] // (2 if call == "gated" else 1)), generator=torch.Generator().manual_seed(1)).bfloat16()
+    grads = []
+    for change in (False, True):
+        rows, weight = x.clone(), w1.clone()
+        (rows if frozen == "weight" else weight).requires_grad_()
+        given = rows * 1                       # (a leaf that needs a gradient is not written in place)
+        y = getattr(experts, call)(given, weight, num)
+        if change:
+            with torch.no_grad():
+                (given if frozen == "weight" else weight).zero_()
+        y.backward(grad_y)
+        grads.append(rows.grad if frozen == "weight" else weight.grad)
+    assert grads[0].float().abs().sum() > 0 and torch.equal(*grads)
+
+
+@pytest.mark.parametrize("call", ["matmul", "gated"])
+def test_rows_rewritten_before_backward_are_an_error(call):
+    x, w1, _, num, _ = _operands((2, 3))
+    given = x.clone()
+    y = getattr(experts, call)(given, w1.requires_grad_(), num)
+    given.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
