@@ -322,6 +322,17 @@ const Tensor *scales_of(PyObject *obj, const char *name) {
     return t;
 }
 
+// What the library writes is written past torch.  Raising the tensor's version, as an operation in place does, lets autograd refuse a
+// backward pass that would read it as it was before.  (Inference tensors have no version, nor a backward pass.)  Done behind the launch,
+// whatever the call returns, and beside what it launched.
+void written(const Tensor *t) {
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+void written(PyObject *obj) {
+    if (obj != nullptr && obj != Py_None) written(&THPVariable_Unpack(obj));
+}
+
 bool has_shape(const Tensor &t, int64_t rows, int64_t cols) { return t.size(0) == rows && t.size(1) == cols; }
 
 uint64_t row_bytes(const Tensor &t) { return (uint64_t)t.stride(0) * t.element_size(); }
@@ -561,6 +572,9 @@ PyObject *dispatch(Operator *op, PyObject *const *args, Py_ssize_t n, PyObject *
         Py_BEGIN_ALLOW_THREADS
         rc = a2a_dispatch(ctx, step.args, (uint32_t)quantize, stream);
         Py_END_ALLOW_THREADS
+        for (uint32_t r = 0; r < op->world; ++r) {
+            for (int i = 0; i < 3; ++i) written(step.kept[r][i]);   // counts, rows, scales
+        }
         if (rc != 0) return raise_last_error(ctx, "a2a_dispatch", rc);
         Py_RETURN_NONE;
     }
@@ -579,6 +593,11 @@ PyObject *dispatch(Operator *op, PyObject *const *args, Py_ssize_t n, PyObject *
                                d.out_x_scale_stride_elem, d.out_x_scale_stride_token, stream);
     }
     Py_END_ALLOW_THREADS
+    if (do_recv) {
+        written(out_n);
+        written(out_x);
+        written(out_scale);
+    }
     if (rc != 0) return raise_last_error(ctx, do_send ? "a2a_dispatch_send" : "a2a_dispatch_recv", rc);
     Py_RETURN_NONE;
 }
@@ -654,6 +673,7 @@ PyObject *combine(Operator *op, PyObject *const *args, Py_ssize_t n, PyObject *k
         Py_BEGIN_ALLOW_THREADS
         rc = a2a_combine(ctx, step.args, (uint32_t)y_tag, (uint32_t)accumulate, stream);
         Py_END_ALLOW_THREADS
+        for (uint32_t r = 0; r < op->world; ++r) written(step.kept[r][0]);
         if (rc != 0) return raise_last_error(ctx, "a2a_combine", rc);
         Py_RETURN_NONE;
     }
@@ -681,6 +701,7 @@ PyObject *combine(Operator *op, PyObject *const *args, Py_ssize_t n, PyObject *k
                               (uint32_t)accumulate, stream);
     }
     Py_END_ALLOW_THREADS
+    if (do_recv) written(out);
     if (rc != 0) return raise_last_error(ctx, do_send ? "a2a_combine_send" : "a2a_combine_recv", rc);
     Py_RETURN_NONE;
 }
@@ -958,6 +979,9 @@ PyObject *expert_forward(bool gated, PyObject *const *a) {
     }
     void *const stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)all.device).stream();
     const int rc = gated ? a2a_expert_gated(&p, stream) : a2a_expert_matmul(&p, stream);
+    written(out);
+    written(out_scale);
+    written(projections);
     if (rc != 0) return raise_last_error(nullptr, gated ? "a2a_expert_gated" : "a2a_expert_matmul", rc);
     Py_RETURN_NONE;
 }
@@ -1025,6 +1049,9 @@ PyObject *expert_gradient(bool gated, PyObject *const *a) {
     p.weight_stride_expert = experts > 1 ? (uint64_t)w->stride(0) * w->element_size() : 0;
     void *const stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)all.device).stream();
     const int rc = gated ? a2a_expert_gated_grad(&p, stream) : a2a_expert_matmul_grad(&p, stream);
+    written(a[0]);
+    written(a[1]);
+    if (gated) written(a[2]);
     if (rc != 0) return raise_last_error(nullptr, gated ? "a2a_expert_gated_grad" : "a2a_expert_matmul_grad", rc);
     Py_RETURN_NONE;
 }

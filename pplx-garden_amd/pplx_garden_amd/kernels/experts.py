@@ -15,7 +15,10 @@ with rows and weights in
   float16 or float32, what `combine()` reads; `expert_gated` writes float8_e4m3fn and `out_scale`, quantised as dispatch quantises,
   which the next `expert_matmul` reads.
 * `bfloat16` or `float16`: `out` has the same type, and there are gradients.  `matmul` and `gated` are the same
-  products for autograd.
+  products for autograd.  Where the weight needs a gradient, `expert_x` has to stay as it was until backward: a receive buffer that the next
+  `dispatch()` writes before that makes backward raise, as an operation in place does (every call of the operator and of this module
+  raises the versions of the tensors it writes; replays of a graph and calls on bare addresses do not).  The counts may
+  change, backward has a copy.
 
 Calls enqueue kernels on the current stream of the tensors' GPU, read the counts on the GPU and can be captured into a
 graph.  They allocate nothing but, where the buffer has up to 512 rows, 16 MiB of the stream's own for sums in parts.
