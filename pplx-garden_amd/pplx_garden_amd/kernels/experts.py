@@ -112,12 +112,15 @@ def _save_for_backward(ctx, expert_x, weight, num, padding, *more) -> None:
 
 
 def _gradients(ctx, grad_out):
-    """Memory for both gradients (None: not asked for), the operands, and what else was saved.  In the place of an operand that was not
-    kept stands the gradient that is as large: the calls do not read its values."""
+    """Memory for both gradients (None: not asked for), the gradient they come from, the operands, and what else was saved.  In the place
+    of an operand that was not kept stands the gradient that is as large: the calls do not read its values."""
+    grad_out = grad_out.contiguous()
+    if grad_out.data_ptr() % 16 != 0:   # (a part of a longer gradient may begin anywhere)
+        grad_out = grad_out.clone()
     expert_x, weight, *more = ctx.saved_tensors
     grad_x = grad_out.new_zeros(ctx.shapes[0]) if ctx.needs_input_grad[0] else None
     grad_w = grad_out.new_empty(ctx.shapes[1]) if ctx.needs_input_grad[1] else None
-    return grad_x, grad_w, grad_x if expert_x is None else expert_x, grad_w if weight is None else weight, *more
+    return grad_x, grad_w, grad_out, grad_x if expert_x is None else expert_x, grad_w if weight is None else weight, *more
 
 
 class _Matmul(torch.autograd.Function):
@@ -132,8 +135,8 @@ class _Matmul(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        grad_x, grad_w, expert_x, weight, num = _gradients(ctx, grad_out)
-        expert_matmul_grad(grad_x, grad_w, grad_out.contiguous(), expert_x, weight, num, ctx.expert_padding)
+        grad_x, grad_w, grad_out, expert_x, weight, num = _gradients(ctx, grad_out)
+        expert_matmul_grad(grad_x, grad_w, grad_out, expert_x, weight, num, ctx.expert_padding)
         return grad_x, grad_w, None, None, None
 
 
@@ -150,8 +153,8 @@ class _Gated(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        grad_x, grad_w, expert_x, weight, num, projections = _gradients(ctx, grad_out)
-        expert_gated_grad(grad_x, grad_w, torch.empty_like(projections), grad_out.contiguous(), projections, expert_x, weight,
+        grad_x, grad_w, grad_out, expert_x, weight, num, projections = _gradients(ctx, grad_out)
+        expert_gated_grad(grad_x, grad_w, torch.empty_like(projections), grad_out, projections, expert_x, weight,
                           num, ctx.expert_padding)
         return grad_x, grad_w, None, None, None
 

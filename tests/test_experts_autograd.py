@@ -125,3 +125,21 @@ def test_rows_rewritten_before_backward_are_an_error(call):
     given.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("call", ["matmul", "gated"])
+def test_a_gradient_that_autograd_cuts_out_of_a_longer_one(call):
+    """The result flattened behind a few other values: its gradient is whole rows, but begins at any multiple of two bytes."""
+    x, w1, _, num, _ = _operands((2, 3))
+    grads = []
+    for joined in (False, True):
+        rows, weight = x.clone().requires_grad_(), w1.clone().requires_grad_()
+        y = getattr(experts, call)(rows, weight, num)
+        c = torch.randn(y.shape, generator=torch.Generator().manual_seed(2)).bfloat16()
+        if joined:
+            torch.cat([y.new_zeros(3), y.flatten()]).backward(torch.cat([c.new_zeros(3), c.flatten()]))
+        else:
+            y.backward(c)
+        grads.append((rows.grad, weight.grad))
+    for a, b in zip(*grads):
+        assert a.float().abs().sum() > 0 and torch.equal(a, b)

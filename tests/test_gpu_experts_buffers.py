@@ -144,3 +144,28 @@ def test_a_second_dispatch_into_the_rows_of_a_pending_backward_is_found_out(laye
     y.backward(torch.ones_like(y))
     for got, expected in zip((x.grad, k["up"].grad, k["down"].grad), want):
         assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize("call", ["matmul", "gated"])
+def test_a_gradient_that_begins_at_any_address(call):
+    """autograd hands over a part of a longer gradient: whole rows, behind three other values."""
+    from pplx_garden_amd.kernels import experts
+    gen = torch.Generator(device=device())
+    gen.manual_seed(3)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=gen, device=device()).bfloat16()
+
+    x, w, num = normal(5, 24), normal(2, 32, 24), torch.tensor([2, 3], dtype=torch.int32, device=device())
+    c = normal(5, 32 if call == "matmul" else 16)
+    grads = []
+    for joined in (False, True):
+        rows, weight = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = getattr(experts, call)(rows, weight, num)
+        if joined:
+            torch.cat([y.new_zeros(3), y.flatten()]).backward(torch.cat([c.new_zeros(3), c.flatten()]))
+        else:
+            y.backward(c)
+        grads.append((rows.grad, weight.grad))
+    for a, b in zip(*grads):
+        assert a.float().abs().sum() > 0 and torch.equal(a, b)
