@@ -86,6 +86,7 @@ def expert_gated_grad(grad_x: Optional[torch.Tensor], grad_weight: Optional[torc
                                                 expert_num_tokens, expert_padding)
 
 
+@torch.no_grad()
 def quantize_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Weights [experts, n, k] as float8_e4m3fn codes and a float scale per 128 x 128 block: once, when a model is
     loaded.  Same rule as dispatch's for rows: scale = amax / 448, amax at least 1e-4."""

@@ -143,3 +143,13 @@ def test_a_gradient_that_autograd_cuts_out_of_a_longer_one(call):
         grads.append((rows.grad, weight.grad))
     for a, b in zip(*grads):
         assert a.float().abs().sum() > 0 and torch.equal(a, b)
+
+
+def test_quantized_parameters_keep_no_graph():
+    """A model's weights are parameters: their codes are constants, and the float copies behind them are gone."""
+    weight = torch.nn.Parameter(_operands()[1].float())
+    codes, scale = experts.quantize_weight(weight)
+    for t in (codes, scale):
+        assert not t.requires_grad and t.grad_fn is None
+    for got, want in zip((codes, scale), experts.quantize_weight(weight.detach())):
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
