@@ -794,14 +794,14 @@ PyObject *call_without_a_frame(PyObject *, PyObject *function) {
 // ---------------------------------------------------------------------------
 // The experts' products: functions of tensors, without a context.
 // ---------------------------------------------------------------------------
-// A positive number of 31 bits (None: 0).
-bool small_number(PyObject *obj, const char *name, uint32_t *out) {
+// A number of 31 bits from `least` on (None: 0).
+bool small_number(PyObject *obj, const char *name, long long least, uint32_t *out) {
     *out = 0;
     if (obj == Py_None) return true;
     const long long v = PyLong_AsLongLong(obj);
     if (v == -1 && PyErr_Occurred()) return false;
-    if (v < 1 || v > 0x7FFFFFFF) {
-        PyErr_Format(PyExc_ValueError, "%s must be in [1, 2^31), got %lld", name, v);
+    if (v < least || v > 0x7FFFFFFF) {
+        PyErr_Format(PyExc_ValueError, "%s must be in [%lld, 2^31), got %lld", name, least, v);
         return false;
     }
     *out = (uint32_t)v;
@@ -897,9 +897,11 @@ PyObject *expert_forward(bool gated, PyObject *const *a) {
     PyObject *const padding = a[gated ? 8 : 6], *const expected = a[gated ? 9 : 7];
     a2a_expert_args p = {};
     p.struct_size = sizeof p;
-    if (!small_number(padding, "expert_padding", &p.expert_padding) ||
-        !small_number(expected, "tokens_per_expert", &p.rows_per_expert))
+    if (!small_number(padding, "expert_padding", 1, &p.expert_padding) ||
+        !small_number(expected, "tokens_per_expert", 0, &p.rows_per_expert))
         return nullptr;
+    // (less than a row an expert, rounded down; 0 in the structure would be the default)
+    if (expected != Py_None && p.rows_per_expert == 0) p.rows_per_expert = 1;
     A2A_REQUIRE(padding != Py_None);
     ExpertTensors all;
     const Tensor *x = all.take(a[1], "expert_x", 2);
@@ -991,7 +993,7 @@ PyObject *expert_gradient(bool gated, PyObject *const *a) {
     PyObject *const *rest = a + (gated ? 5 : 3);
     a2a_expert_grad_args p = {};
     p.struct_size = sizeof p;
-    if (!small_number(rest[3], "expert_padding", &p.expert_padding)) return nullptr;
+    if (!small_number(rest[3], "expert_padding", 1, &p.expert_padding)) return nullptr;
     A2A_REQUIRE(rest[3] != Py_None);
     ExpertTensors all;
     const Tensor *x = all.take(rest[0], "expert_x", 2);

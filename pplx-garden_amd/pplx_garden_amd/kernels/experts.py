@@ -22,8 +22,8 @@ with rows and weights in
 
 Calls enqueue kernels on the current stream of the tensors' GPU, read the counts on the GPU and can be captured into a
 graph.  They allocate nothing but, where the buffer has up to 512 rows, 16 MiB of the stream's own for sums in parts.
-`tokens_per_expert` is how many rows the caller expects an expert to have (default: rows of the buffer per expert): it
-chooses between kernels, any counts give right results.
+`tokens_per_expert` is how many rows the caller expects an expert to have (default: rows of the buffer per expert; 0 is
+less than one): it chooses between kernels, any counts give right results.
 """
 
 from __future__ import annotations

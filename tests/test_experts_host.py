@@ -173,3 +173,16 @@ def test_the_reference_gradients_are_those_of_the_reference_forward():
 def test_ranges_of_experts():
     assert ref.ranges([3, 0, 5], 4, 20) == [(0, 3), (4, 0), (4, 5)]
     assert ref.ranges([3, 9, 5], 4, 10) == [(0, 3), (4, 6), (10, 0)]
+
+
+def test_a_step_that_expects_less_than_a_row_an_expert_says_none():
+    """tokens * topk // experts of a small step: taken (what the call then refuses is that there is no GPU)."""
+    x, w, num = torch.zeros((4, 16)).bfloat16(), torch.zeros((2, 8, 16)).bfloat16(), torch.zeros(2, dtype=torch.int32)
+    for expected in (0, 1, None):
+        with pytest.raises(AssertionError, match="GPU"):
+            experts.expert_matmul(torch.zeros((4, 8)).bfloat16(), x, w, num, tokens_per_expert=expected)
+        with pytest.raises(AssertionError, match="GPU"):
+            experts.expert_gated(torch.zeros((4, 4)).bfloat16(), x, w, num, tokens_per_expert=expected)
+    for expected in (-1, 1 << 31):
+        with pytest.raises(ValueError, match="tokens_per_expert"):
+            experts.expert_matmul(torch.zeros((4, 8)).bfloat16(), x, w, num, tokens_per_expert=expected)

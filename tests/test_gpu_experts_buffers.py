@@ -169,3 +169,19 @@ def test_a_gradient_that_begins_at_any_address(call):
         grads.append((rows.grad, weight.grad))
     for a, b in zip(*grads):
         assert a.float().abs().sum() > 0 and torch.equal(a, b)
+
+
+def test_a_hint_of_no_rows_is_one_of_the_fewest():
+    from pplx_garden_amd.kernels.experts import expert_gated, expert_matmul
+    gen = torch.Generator(device=device())
+    gen.manual_seed(4)
+    x, w = (torch.randn(s, generator=gen, device=device()).bfloat16() for s in ((40, 64), (4, 32, 64)))
+    num = torch.tensor([0, 1, 0, 2], dtype=torch.int32, device=device())
+    got = []
+    for expected in (0, 1):
+        y, h = (torch.zeros((40, n), device=device()).bfloat16() for n in (32, 16))
+        expert_matmul(y, x, w, num, tokens_per_expert=expected)
+        expert_gated(h, x, w, num, tokens_per_expert=expected)
+        got.append((y, h))
+    for a, b in zip(*got):
+        assert a.float().abs().sum() > 0 and torch.equal(a, b)
