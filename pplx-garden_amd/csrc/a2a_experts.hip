@@ -69,7 +69,8 @@ int units_of(const char *call, int device, uint32_t *units) {
     if (*units != 0) return A2A_OK;
     int count = 0;
     const hipError_t e = hipDeviceGetAttribute(&count, hipDeviceAttributeMultiprocessorCount, device);
-    if (e != hipSuccess || count <= 0) return fail_call((int)e, "%s: hipDeviceGetAttribute: %s", call, hipGetErrorString(e));
+    if (e != hipSuccess) return fail_call((int)e, "%s: hipDeviceGetAttribute: %s", call, hipGetErrorString(e));
+    if (count <= 0) return fail_call(A2A_ERR_UNSUPPORTED, "%s: device %d has %d compute units", call, device, count);
     known[device].store((uint32_t)count, std::memory_order_relaxed);
     *units = (uint32_t)count;
     return A2A_OK;

@@ -3,6 +3,9 @@ definition that the GPU tests compare with."""
 
 import ctypes
 import re
+import shutil
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -186,3 +189,37 @@ def test_a_step_that_expects_less_than_a_row_an_expert_says_none():
     for expected in (-1, 1 << 31):
         with pytest.raises(ValueError, match="tokens_per_expert"):
             experts.expert_matmul(torch.zeros((4, 8)).bfloat16(), x, w, num, tokens_per_expert=expected)
+
+
+RUNTIME_WITHOUT_UNITS = """
+extern "C" {
+int hipGetDevice(int *device) { *device = 0; return 0; }
+int hipSetDevice(int) { return 0; }
+int hipDeviceGetAttribute(int *value, int, int) { *value = 0; return 0; }
+}
+"""
+
+CALL_WITHOUT_UNITS = """
+import ctypes, sys
+sys.path[:0] = sys.argv[2:]
+ctypes.CDLL(sys.argv[1], ctypes.RTLD_GLOBAL)     # before the library: its calls of the runtime find these first
+import test_experts_host as t
+lib = t.native.load_library()
+for call, args in ((lib.a2a_expert_matmul, t.forward()), (lib.a2a_expert_matmul_grad, t.gradient())):
+    print(call(ctypes.byref(args), None), lib.a2a_last_error(None).decode())
+"""
+
+
+def test_a_device_that_names_no_compute_units_is_an_error(tmp_path):
+    """The runtime answers, but with 0 units: refused before anything is launched, with a code that is not success."""
+    compiler = shutil.which("g++") or shutil.which("c++")
+    if compiler is None:
+        pytest.skip("needs a C++ compiler")
+    (tmp_path / "runtime.cpp").write_text(RUNTIME_WITHOUT_UNITS)
+    runtime = tmp_path / "runtime.so"
+    subprocess.run([compiler, "-shared", "-fPIC", str(tmp_path / "runtime.cpp"), "-o", str(runtime)], check=True)
+    here = Path(__file__).resolve().parent
+    result = subprocess.run([sys.executable, "-c", CALL_WITHOUT_UNITS, str(runtime), str(here), str(here.parent / "pplx-garden_amd")],
+                            check=True, capture_output=True, text=True, timeout=100)
+    lines = result.stdout.splitlines()
+    assert len(lines) == 2 and all(line.startswith("-3 ") and "compute units" in line for line in lines), lines
