@@ -47,7 +47,8 @@ struct Run {
 
 // 16 (or 4) bytes a lane from memory into LDS at `lds` + AT + lane * 16 (4); `lds` is the same in all lanes.  Nothing returns to
 // registers, and the compiler does not count these loads: wait_stage() does.  (One wait state lies between a write of m0
-// and the load that uses it.)
+// and the load that uses it.  m0 cannot be named as overwritten, it is reserved; the compiler's own code does not use it in these kernels,
+// which a test looks at.)
 // ONCE: of memory that nobody reads again, past the caches.
 template <int AT, bool ONCE>
 __device__ __forceinline__ void load_to_lds16(uint32_t lds, u32x4 run, uint32_t lane_offset, uint32_t offset) {

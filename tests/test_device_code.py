@@ -1,5 +1,6 @@
 """What the compiler cannot check in the device code (CPU: hipcc cross-compiles)."""
 
+import importlib
 import re
 import shutil
 import subprocess
@@ -71,3 +72,20 @@ def test_limits_that_packed_words_do_not_hold_are_refused(tmp_path, limit, large
     result = subprocess.run(cmd, capture_output=True, text=True)
     assert (result.returncode == 0) == (refused is None), result.stderr
     assert refused is None or refused in result.stderr
+
+
+@pytest.mark.skipif(not Path(HIPCC).exists(), reason="needs hipcc")
+def test_the_compiler_keeps_nothing_in_m0():
+    """The experts' products write m0 in inline assembly, which cannot name it: it is reserved, and the compiler warns of it in a list of
+    what is overwritten.  So the compiler's own code must not use it in these kernels."""
+    flags = [*importlib.import_module("build").HIPCC_FLAGS, "-I", str(ROOT.parent / "include"), "-I", str(ROOT / "csrc")]
+    runs = [subprocess.Popen([HIPCC, *flags, "-S", "--offload-device-only", str(ROOT / "csrc" / name), "-o", "-"],
+                             stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, text=True)
+            for name in ("a2a_experts_forward.hip", "a2a_experts_gradient.hip")]
+    for run in runs:
+        assembly = run.communicate()[0]
+        assert run.returncode == 0
+        ours = re.findall(r"#ASMSTART(.*?)#ASMEND", assembly, re.S)
+        assert sum("m0" in block for block in ours) > 100
+        rest = re.sub(r"#ASMSTART.*?#ASMEND", "", assembly, flags=re.S)
+        assert "s_endpgm" in rest and not re.search(r"\bm0\b", rest)
