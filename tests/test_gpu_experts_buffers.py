@@ -185,3 +185,35 @@ def test_a_hint_of_no_rows_is_one_of_the_fewest():
         got.append((y, h))
     for a, b in zip(*got):
         assert a.float().abs().sum() > 0 and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("arguments", [[], ["--padding", "16", "--tokens", "37", "--inter", "264"]])
+def test_the_gradients_of_the_examples_training_step(arguments):
+    """Of the rows and of both weights, rank by rank, against the layer's derivative in 64 bits on the rows that dispatch has left.  Every rounding
+    to bfloat16 is one of 2^-8 at most: gates, ups, the gradient of the block, that of the projections and the result of the rows and of the
+    first weights; the block and the result of the second weights."""
+    import experts_reference as ref
+    example = _example()
+    a = example.parse(["--train", *arguments])
+    ranks, _, _ = example.make_layer(a, device(), fp8=False)
+    gen = torch.Generator(device=device())
+    gen.manual_seed(5)
+    grad_y = [torch.randn(k["y"].shape, generator=gen, device=device()).bfloat16() for k in ranks]
+    example.train(a, ranks, grad_y)
+    for k, c in zip(ranks, grad_y):
+        rows, up, down = (t.detach().double() for t in (k["rows"], k["up"], k["down"]))
+        got = dict(rows=k["grad_rows"], up=k["up"].grad, down=k["down"].grad)
+        want = dict(rows=torch.zeros_like(rows), up=torch.zeros_like(up), down=torch.zeros_like(down))
+        for e, (first, count) in enumerate(ref.ranges(k["num"].tolist(), a.padding, rows.shape[0])):
+            at = slice(first, first + count)
+            g, u = (rows[at] @ up[e].T).chunk(2, -1)
+            dy = c[at].double()
+            want["down"][e] = dy.T @ (ref.silu(g) * u)
+            d = torch.cat(ref.gate_gradient(dy @ down[e], g, u), -1)
+            want["rows"][at], want["up"][e] = d @ up[e], d.T @ rows[at]
+        for name, roundings in (("rows", 5), ("up", 5), ("down", 2)):
+            off = (got[name].double() - want[name]).norm() / want[name].norm()
+            assert off < roundings * 2.0 ** -8, (name, off.item())
+        assert not got["rows"][want["rows"].abs().sum(1) == 0].any()
+        assert not got["up"][k["num"] == 0].any() and not got["down"][k["num"] == 0].any()
+        k["op"].destroy()
