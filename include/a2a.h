@@ -378,7 +378,9 @@ typedef struct a2a_expert_args {
     uint32_t expert_padding;         /* each expert's range of rows is rounded up to this */
     uint32_t rows;                   /* rows of x and out */
     uint32_t rows_per_expert;        /* what the caller expects an expert to have, 0: rows / num_experts.  Chooses
-                                        the tile; results do not depend on it beyond the order of the sums */
+                                        the tile (sums in parts, the narrow tile of the smallest steps and whether
+                                        weights are kept in the caches go by `rows`); results do not depend on it
+                                        beyond the order of the sums */
     uint32_t n;                      /* columns of out */
     uint32_t k;                      /* columns of x and of the weights */
     uint32_t in_dtype;               /* a2a_scalar_type of x and the weights */
@@ -425,7 +427,8 @@ int a2a_expert_gated(const a2a_expert_args *args, void *stream);
  *                            then dx and dW from it
  *
  * Either of grad_x and grad_weight may be NULL.  The weight of an expert without
- * rows gets a gradient of zero.  Row strides are as above.
+ * rows gets a gradient of zero.  Row strides are as above.  The tiles go by
+ * rows / num_experts.
  */
 typedef struct a2a_expert_grad_args {
     uint32_t struct_size;            /* sizeof(a2a_expert_grad_args) */

@@ -17,7 +17,7 @@ enum ProductEnd : int {
     kPlain = 0,      // the sums, rounded to the output's type
     kGated = 1,      // silu of the first half of the columns times the second half, and the projections themselves
     kGatedFp8 = 2,   // the same product in e4m3 with a scale per 128 columns
-    kPartial = 3     // sums over parts of the operands' length, in float, for launch_finish to add up
+    kPartial = 3     // sums over parts of the operands' length, in float, for finish_kernel to add up
 };
 
 struct ProductArgs {
