@@ -88,7 +88,8 @@ def serve(a, ranks):
 
 
 def train(a, ranks, grad_y):
-    """The same with gradients: `grad_y` is what the loss makes of every rank's expert rows."""
+    """The same with gradients: `grad_y` is what the loss makes of every rank's expert rows.  The products read the receive buffer itself, so
+    backward comes before the next dispatch into it (which would make it raise)."""
     dispatch(ranks)
     for k, g in zip(ranks, grad_y):
         x = k["rows"].detach().requires_grad_()

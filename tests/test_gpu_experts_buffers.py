@@ -217,3 +217,33 @@ def test_the_gradients_of_the_examples_training_step(arguments):
         assert not got["rows"][want["rows"].abs().sum(1) == 0].any()
         assert not got["up"][k["num"] == 0].any() and not got["down"][k["num"] == 0].any()
         k["op"].destroy()
+
+
+@pytest.mark.parametrize("call", ["matmul", "gated"])
+def test_gradients_with_the_rows_or_the_weight_frozen(call):
+    """The operand that is not read is not kept, and may have changed by then; no rows at all are a gradient of zeros."""
+    from pplx_garden_amd.kernels import experts
+    gen = torch.Generator(device=device())
+    gen.manual_seed(6)
+    x, w = (torch.randn(s, generator=gen, device=device()).bfloat16() for s in ((300, 72), (3, 48, 72)))
+    num = torch.tensor([100, 0, 200], dtype=torch.int32, device=device())
+    c = torch.randn((300, 48 if call == "matmul" else 24), generator=gen, device=device()).bfloat16()
+
+    product = getattr(experts, call)
+    rows, weight = x.clone().requires_grad_(), w.clone().requires_grad_()
+    product(rows, weight, num).backward(c)
+    want = rows.grad, weight.grad
+    assert all(g.float().abs().sum() > 0 for g in want)
+    weight = w.clone().requires_grad_()
+    product(x, weight, num).backward(c)
+    assert torch.equal(weight.grad, want[1])
+    rows = x.clone().requires_grad_()
+    given = rows * 1
+    y = product(given, w, num)
+    experts.expert_matmul(given.detach(), c.new_zeros((300, 8)), c.new_zeros((3, 72, 8)), num)   # writes the rows again
+    assert not given.any()
+    y.backward(c)
+    assert torch.equal(rows.grad, want[0])
+    weight.grad = None
+    product(x[:0], weight, torch.zeros_like(num)).backward(c[:0])
+    assert weight.grad.shape == w.shape and not weight.grad.any()
